@@ -16,7 +16,6 @@ c + i of the sequence's block table.
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -201,9 +200,7 @@ def _rows(g: torch.Generator, cache: str, slots: int, kv_heads: int, d: int):
     return data, scale
 
 
-@functools.cache
 def _package():
-    """The framework's modules, imported once as a program does."""
     path = str(Path(__file__).resolve().parent.parent / "llm-serving-engine_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
