@@ -264,10 +264,40 @@ __global__ __launch_bounds__(kSliceThreads) void row_stats_kernel(VerifyArgs a) 
   slice_of_row(a.logits + t * a.V, a.V, blockIdx.y, greedy, temp, a.stats + t * a.slices);
 }
 
+// What the tokens of the lanes in `struck` leave of a row's softmax, for a whole wavefront: a sum over all others.
+__device__ __forceinline__ double mass_of(const float* row, int64_t V, int64_t tok, uint64_t struck, float c, float top, float inv_z) {
+  constexpr int N = 4;
+  double sum = 0.0;
+  for (int64_t base = 0; base < V; base += 4 * N * kWave) {
+    const int64_t v0 = base + 4 * (threadIdx.x % kWave);
+    f32x4u x[N];
+    block_of<N, kWave>(row, base, v0, V, -__builtin_inff(), x);
+    for (uint64_t todo = __ballot(tok >= base && tok < base + 4 * N * kWave) & struck; todo; todo &= todo - 1) {
+      const int64_t at = __shfl(static_cast<long long>(tok), __builtin_ctzll(todo), kWave) - v0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = at == 4 * kWave * i + e ? -__builtin_inff() : x[i][e];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += static_cast<double>(__builtin_amdgcn_exp2f((x[i][e] - top) * c)) * inv_z;
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d, kWave);
+  return sum;
+}
+
 // A lane's node as the tests of given drafts see it: `child` of the node, its token (-1: none), number and
-// probability. The first of `children` that is accepted, or -1; `struck`: the rejected ones, whose tokens are
-// out.
-__device__ __forceinline__ int take_given(uint64_t children, bool child, int64_t tok, float unif, double p_own, uint64_t& struck) {
+// probability (exp2((logit - top) c) inv_z of the node's row). The first of `children` that is accepted, or -1;
+// `struck`: the rejected ones, whose tokens are out.
+// What is left of p is 1 less the struck tokens' p, while that is far from their roundings (under 2^-20 together);
+// below kSure it is summed: a walk gets there with a probability of no more than kSure. So a token that has all that is
+// left has r = 1 and is taken, and one that is not 0 remains for the race.
+constexpr double kSure = 0x1p-14;
+__device__ __forceinline__ int take_given(uint64_t children, bool child, int64_t tok, float unif, double p_own, const float* row,
+                                          int64_t V, float c, float top, float inv_z, uint64_t& struck) {
   double left = 1.0;  // what the struck tokens left of p
   struck = 0;
   for (uint64_t todo = children; todo; todo &= todo - 1) {
@@ -276,10 +306,15 @@ __device__ __forceinline__ int take_given(uint64_t children, bool child, int64_t
     const int64_t t = __shfl(static_cast<long long>(tok), i, kWave);
     const bool again = (__ballot(child && tok == t) & struck) != 0;  // struck already
     if (number < (again ? 0.0 : p / left)) return i;
-    if (t >= 0 && p > 0.0 && !again && left - p > 0.0) {
-      left -= p;
-      struck |= 1ull << i;
+    if (t < 0 || !(p > 0.0) || again) continue;
+    double rest = left - p;
+    if (rest < kSure) rest = mass_of(row, V, tok, struck | 1ull << i, c, top, inv_z);
+    if (!(rest > 0.0)) {  // the token has all of it
+      if (number < 1.0) return i;
+      continue;
     }
+    left = rest;
+    struck |= 1ull << i;
   }
   return -1;
 }
@@ -314,7 +349,8 @@ __global__ __launch_bounds__(kSliceThreads) void level_kernel(VerifyArgs a, int 
         const float inv_z = 1.f / sum;
         uint64_t struck;
         node = take_given(children, child, tok, unif,
-                          tok >= 0 ? static_cast<double>(__builtin_amdgcn_exp2f((xl - top) * c)) * inv_z : 0.0, struck);
+                          tok >= 0 ? static_cast<double>(__builtin_amdgcn_exp2f((xl - top) * c)) * inv_z : 0.0,
+                          a.logits + (u.first + before) * a.V, a.V, c, top, inv_z, struck);
       }
     }
   }
@@ -488,7 +524,8 @@ __device__ __forceinline__ State walk(const VerifyArgs& a, int s, Shared<WAVES>&
       st.inv_z = inv_z;
       st.struck = 0;
       st.c = st.c_before = 0.f;
-      if (a.probs == nullptr) taken = take_given(children, par == node, tok, unif, p_own, st.struck);
+      if (a.probs == nullptr)
+        taken = take_given(children, par == node, tok, unif, p_own, a.logits + (u.first + node) * a.V, a.V, c, top, inv_z, st.struck);
       double rc = 0.0, rn = 1.0;  // drawn drafts: r = (p - rc q)+ / rn
       for (uint64_t todo = PASSES && a.probs ? children : 0; todo && taken < 0; todo &= todo - 1) {
         const int i = __builtin_ctzll(todo);

@@ -1,0 +1,68 @@
+"""Verification steps over drafted trees on the GPU, where arithmetic is at its limits: drafts that cover all
+of a row, logits far from 0, channels of very different size beside each other, batches of large and small trees.
+
+Tolerances are those of ``test_gpu_speculative.py`` unless a test derives its own.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from llmserve import speculative as sp
+from spec_util import Batch, check_walks, random_tree
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+NEAR = 2e-5
+UNDER_ONE = F32(1 - 2.0 ** -24)  # the largest uniform number
+
+
+# ---- drafts that cover a row ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seqs,v,max_depth", [(40, 4099, 63), (1600, 4099, 3), (90, 262147, 3), (90, 262147, 63)])
+def test_siblings_that_cover_a_row(gpu, seqs, v, max_depth):
+    """Two or three tokens have all of a row's mass and all are drafted, or all but one: a first token may have
+    all but 2^-20 of it. With uniform numbers just below 1 every child but the last is rejected; the last
+    one's r is 1, so it is kept; where one token is not drafted, that is the next token. The walks in the race's
+    launch, in one of their own, after launches for a path's nodes, and by workgroups that read rows."""
+    rng = np.random.default_rng(seqs)
+    trees = [[-1] + [0] * (2 if i % 3 else 3) for i in range(seqs)]
+    b = Batch(41, [2] * seqs, trees, 16, gpu, max_nodes=max_depth + 1)
+    if v > 200000:
+        assert b.T * v > 75 << 20  # rows too many to be read ahead of the walks
+    x = torch.full((b.T, v), -float("inf"), device=gpu)
+    tokens, want, set_at = np.zeros(b.T, np.int64), [], []
+    for i, tree in enumerate(trees):
+        a, kids = int(b.start[i]), len(tree) - 1
+        support = rng.choice(v, 3 if i % 3 != 1 else 2, replace=False)
+        # below e^-13.31 of the first: the rest of 1 is under 1.7e-6, rounded as 1 is; else shares of a few per cent and more
+        first = 13.31 if i % 2 else rng.random() * 2
+        low = [0.0] + [first + rng.random() for _ in support[1:]]
+        set_at += [(a, int(t), -y) for t, y in zip(support, low)]
+        end = int(rng.integers(v))
+        set_at += [(a + j, end, 1.0) for j in range(1, kids + 1)]
+        tokens[a + 1: a + 1 + kids] = support[:kids]
+        covered = kids == len(support)
+        want.append(([0, kids], [int(support[kids - 1]), end]) if covered else ([0], [int(support[-1])]))
+    rows, at, values = (np.array(z) for z in zip(*set_at))
+    x[torch.from_numpy(rows).to(gpu), torch.from_numpy(at).to(gpu)] = torch.from_numpy(values.astype(F32)).to(gpu)
+    noise = torch.empty(seqs, v, device=gpu).exponential_(generator=torch.Generator(gpu).manual_seed(2))
+    got = sp.verify_draft(x, b.draft, b.put(tokens), torch.ones(seqs, device=gpu), b.put([UNDER_ONE] * b.T, F32), noise)
+    for s, (path, out) in enumerate(want):
+        assert got.accepted[s] == len(path) - 1 and got.path[s, : len(path)].tolist() == path, (s, got.path[s, :4])
+        assert got.tokens[s, : len(out)].tolist() == out, s
+
+
+def test_walks_of_rows_just_too_many_to_read_ahead(gpu):
+    """Between the limits of given and of drawn drafts: a launch for each of a path's nodes."""
+    v, rng = 98511, np.random.default_rng(12)
+    trees = [random_tree(rng, 58) for _ in range(16)]
+    b = Batch(42, [2] * len(trees), trees, 16, gpu, max_depth=8)
+    assert 75 << 20 < b.T * v < 150 << 20
+    x, tokens, u, noise, _ = b.logits(v, lift=0.6)
+    temps = [0.0 if i % 5 == 0 else 0.9 for i in range(len(trees))]
+    got = b.verify(x, tokens, temps, u, noise)
+    assert check_walks(got, b.walks(x, tokens, temps, u, noise, max_depth=8), NEAR) >= len(trees) - 2
