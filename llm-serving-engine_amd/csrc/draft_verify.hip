@@ -21,8 +21,10 @@
 // all CUs share; the walks, a lane for each node, every lane with its own test's numbers in registers; the
 // race for the last token over slices of the last row, as maxima of (key, index) words; their maximum. (A
 // last slice that joins them, by an atomic count, took longer: what the other XCDs wrote has to be made
-// visible to it, 9.7 us against 4 and a launch for one stream.) The race compares log2(e) x / temperature - log2 E,
-// so that it needs no softmax.
+// visible to it, 9.7 us against 4 and a launch for one stream.) The race compares log2(e) (x - m) / temperature - log2 E, m
+// the largest x of a wavefront's part and then of a slice, taken along and made up for where parts are joined: it needs no
+// softmax, and sees no shift of a row, as a softmax does not (without m, logits of 10^4 at temperature 0.01
+// had keys of 10^6, and the noise was rounded off).
 //
 // Many rows (large trees) would be read for nothing: a walk visits a few of a tree's rows. There, the first
 // launch is one for each of the path's first kLevels nodes: every workgroup takes the step from the node
@@ -83,6 +85,7 @@ struct VerifyArgs {
   int64_t *accepted, *path, *tokens;
   State* state;     // [S]
   uint64_t* words;  // [S][slices][2] maxima of the race: after the last rejection, before it
+  float* refs;      // [S][slices] what the first of them are relative to: the slices' largest logits
   Stat* stats;      // [T][slices], or of the first levels' nodes [level][S][slices]; null: the walks read the rows
   int* cursors;     // [level][S] the path's nodes (-1: it ends before); null: rows ahead, or none
   int levels;
@@ -98,7 +101,15 @@ __device__ __forceinline__ uint64_t word_of(float key, uint32_t idx) {
   return static_cast<uint64_t>(order_key(key)) << 32 | ~idx;
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t word) { return ~static_cast<uint32_t>(word); }
+__device__ __forceinline__ float key_of(uint64_t word) {
+  const uint32_t u = static_cast<uint32_t>(word >> 32);
+  return __builtin_bit_cast(float, (u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
 constexpr uint64_t kBad = ~0ull;  // a row whose softmax is not a number
+// A word of the race whose key is relative to a logit `ref`, made relative to one of at least that size.
+__device__ __forceinline__ uint64_t shifted(uint64_t word, float ref, float to, float scale) {
+  return word == 0 || word == kBad || ref == to ? word : word_of(__builtin_fmaf(ref - to, scale, key_of(word)), index_of(word));
+}
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
@@ -631,6 +642,7 @@ template <bool WALK>
 __global__ __launch_bounds__(kSliceThreads) void race_kernel(VerifyArgs a) {
   constexpr int kWaves = kSliceThreads / kWave;
   __shared__ uint64_t words[2][kWaves];
+  __shared__ float tops[kWaves];
   __shared__ Shared<1> none;
   __shared__ State walked;
   __shared__ uint32_t out[kSlice / 32];  // bits: struck tokens of the slice
@@ -671,6 +683,18 @@ __global__ __launch_bounds__(kSliceThreads) void race_kernel(VerifyArgs a) {
     }
     __syncthreads();
   }
+  // the largest logit of the wavefront's part (one that is not finite: 0, and the row is bad or the part empty)
+  float ref = 0.f;
+  if (!drawn) {
+    ref = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ref = fmaxf(ref, x[i][j]);
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) ref = fmaxf(ref, __shfl_xor(ref, d, kWave));
+    ref = fabsf(ref) < __builtin_inff() ? ref : 0.f;
+  }
   // this thread's largest key and its token, the first of equal ones (tokens come in growing order)
   float key = -__builtin_inff(), key_before = -__builtin_inff();
   uint32_t at = 0, at_before = 0;
@@ -695,7 +719,7 @@ __global__ __launch_bounds__(kSliceThreads) void race_kernel(VerifyArgs a) {
         at_before = k0 > key_before ? idx : at_before;
         key_before = fmaxf(key_before, k0);
       } else {
-        const float k = gone >> j & 1 ? -__builtin_inff() : __builtin_fmaf(x[i][j], scale, -lg_e);
+        const float k = gone >> j & 1 ? -__builtin_inff() : __builtin_fmaf(x[i][j] - ref, scale, -lg_e);
         at = k > key ? idx : at;
         key = fmaxf(key, k);
       }
@@ -709,17 +733,23 @@ __global__ __launch_bounds__(kSliceThreads) void race_kernel(VerifyArgs a) {
   if (lane == 0) {
     words[0][tid / kWave] = best;
     words[1][tid / kWave] = before;
+    tops[tid / kWave] = best ? ref : -__builtin_inff();
   }
   __syncthreads();
   if (tid != 0) return;
+  float top_ref = tops[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top_ref = fmaxf(top_ref, tops[w]);
+  best = shifted(best, tops[0], top_ref, scale);
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) {
-    best = max64(best, words[0][w]);
+    best = max64(best, shifted(words[0][w], tops[w], top_ref, scale));
     before = max64(before, words[1][w]);
   }
-  uint64_t* const out_words = a.words + (static_cast<int64_t>(s) * a.slices + blockIdx.x) * 2;
-  out_words[0] = best;
-  out_words[1] = before;
+  const int64_t at_slice = static_cast<int64_t>(s) * a.slices + blockIdx.x;
+  a.words[2 * at_slice] = best;
+  a.words[2 * at_slice + 1] = before;
+  a.refs[at_slice] = top_ref;
 }
 
 // Joins the slices: a wavefront for each sequence.
@@ -728,11 +758,20 @@ __global__ __launch_bounds__(kWave) void finish_kernel(VerifyArgs a) {
   const State* const state = a.state + s;
   if (state->node < 0) return;
   const uint64_t* words = a.words + static_cast<int64_t>(s) * a.slices * 2;
-  uint64_t best = 0, before = 0;
+  const float* refs = a.refs + static_cast<int64_t>(s) * a.slices;
+  const float scale = kLog2e / a.temperature[s];
+  uint64_t best = 0, before = 0;  // of this lane's slices
+  float ref = -__builtin_inff();  // what best is relative to
   for (int i = lane; i < a.slices; i += kWave) {
-    best = max64(best, words[2 * i]);
+    const float other = refs[i], to = fmaxf(ref, other);
+    best = max64(shifted(best, ref, to, scale), shifted(words[2 * i], other, to, scale));
+    ref = to;
     before = max64(before, words[2 * i + 1]);
   }
+  float top = ref;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+  best = shifted(best, ref, top, scale);
   best = wave_max64(best);
   before = wave_max64(before);
   const uint64_t word = best ? best : before;
@@ -747,7 +786,7 @@ int64_t slices_of(int64_t V) { return (V + kSlice - 1) / kSlice; }
 
 extern "C" int64_t llmserve_verify_draft_workspace_bytes(int64_t S, int64_t T, int64_t V) {
   if (S <= 0 || T < 0 || V <= 0) return 0;
-  return S * static_cast<int64_t>(sizeof(State)) + S * slices_of(V) * 16 +
+  return S * static_cast<int64_t>(sizeof(State)) + S * slices_of(V) * (16 + static_cast<int64_t>(sizeof(float))) + 8 +
          std::max(T * V <= kAhead ? T * slices_of(V) * static_cast<int64_t>(sizeof(Stat)) : 0,
                   T * V > kAheadGiven ? kLevels * S * (slices_of(V) * static_cast<int64_t>(sizeof(Stat)) + 4) : 0);
 }
@@ -774,11 +813,12 @@ extern "C" int llmserve_verify_draft(const float* logits, const int64_t* draft_t
   uint64_t* const words = reinterpret_cast<uint64_t*>(state + S);
   const bool ahead = T * V <= (draft_probs ? kAhead : kAheadGiven), by_level = !ahead && draft_probs == nullptr;
   const int levels = static_cast<int>(max_depth + 1 < kLevels ? max_depth + 1 : kLevels);
-  Stat* const stats = reinterpret_cast<Stat*>(words + S * slices * 2);
+  float* const refs = reinterpret_cast<float*>(words + S * slices * 2);
+  Stat* const stats = reinterpret_cast<Stat*>(refs + (S * slices + 1) / 2 * 2);  // (8-byte words in greedy rows)
   const VerifyArgs a{logits, draft_probs, draft_tokens, parents, static_cast<const int*>(plan), temperature, uniforms, noise,
                T, V, static_cast<int>(S), static_cast<int>(max_depth + 1), static_cast<int>(slices),
                accepted, path, tokens, state,
-               words, ahead || by_level ? stats : nullptr,
+               words, refs, ahead || by_level ? stats : nullptr,
                by_level ? reinterpret_cast<int*>(stats + levels * S * slices) : nullptr, levels};
   hipStream_t st = lsh::as_stream(stream);
   const unsigned n = static_cast<unsigned>(S), parts = static_cast<unsigned>(slices);

@@ -66,3 +66,27 @@ def test_walks_of_rows_just_too_many_to_read_ahead(gpu):
     temps = [0.0 if i % 5 == 0 else 0.9 for i in range(len(trees))]
     got = b.verify(x, tokens, temps, u, noise)
     assert check_walks(got, b.walks(x, tokens, temps, u, noise, max_depth=8), NEAR) >= len(trees) - 2
+
+
+# ---- the race far from 0 ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seqs,drawn", [(40, False), (1600, False), (40, True)])
+@pytest.mark.parametrize("offset,temp", [(0.0, 0.01), (1000.0, 0.01), (1e4, 0.01), (-1e4, 1.0), (3e5, 1.0)])
+def test_the_race_does_not_see_a_shift(gpu, seqs, drawn, offset, temp):
+    """Logits around an offset, most of them equal to the largest: the noise decides among those, and a softmax does
+    not change with the offset. The rows hold multiples of 2^-5, so that they are the same numbers in 32 bits
+    with every offset here. The race in the walks' launch and in one of its own, a last slice that is short or empty of
+    likely tokens, rejected drafts."""
+    v, rng = 8192 + 1003, np.random.default_rng(int(abs(offset)) + seqs)
+    trees = [[-1] if i % 2 else [-1, 0, 0] for i in range(seqs)]
+    b = Batch(43, [2] * seqs, trees, 16, gpu, max_nodes=3)
+    x = (offset - np.where(rng.random((b.T, v)) < 0.7, 0, rng.integers(1, 64, (b.T, v))) / 32).astype(F32)
+    x[::5, 8000:] = -np.inf
+    assert (np.diff(np.unique(x[0, :8000])) >= 1 / 32).all()
+    noise = rng.exponential(size=(seqs, v)).astype(F32)
+    tokens, u = rng.integers(0, v, b.T), np.full(b.T, 0.9, F32)
+    probs = np.full((b.T, v), 1 / v, F32) if drawn else None
+    temps = [temp] * seqs
+    got = b.verify(x, tokens, temps, u, noise, probs)
+    assert check_walks(got, b.walks(x, tokens, np.full(seqs, temp, F32), u, noise, probs), NEAR) >= seqs - 4
