@@ -16,11 +16,14 @@
 // being any four groups of the row's), V's is done by byte permutes in registers (int8) or is none
 // at all (fp32: one register is one element). A row's running reference and sum are per-lane scalars.
 //
-// Precision is fp32's. int8: the scores are exact integer products of the codes with q in three signed
-// digits (23 bits of the row's largest); codes of V are exact in fp16, the weights two fp16 pieces after
-// scaling by a power of two (22 bits); scales stay in fp32 on the score and the weight. fp32: fp32
-// matrix instructions (a step's sums formed apart and added once), where trees have more than 32 rows
-// fp16 ones on two pieces of everything. Errors against 64 bits lie between 2e-7 and 4.5e-7 of the 2-norm.
+// Precision. int8: the scores are exact integer products of the codes with q in three signed digits: an element of
+// q' is held to 2^-24 of its row's largest one, and a score to that times the sum of its token's |code| (less than
+// fp32 keeps where the largest elements of q' meet codes near 0 only). Codes of V are exact in fp16, the weights two
+// fp16 pieces after scaling by a power of two (22 bits); scales stay in fp32 on the score and the weight. fp32: fp32
+// matrix instructions (a step's sums formed apart and added once), for a head size of 128 and more than 32 rows a
+// tree on average fp16 ones on two pieces of everything: 22 bits of every element down to 2^-29 of its row's largest.
+// Errors against 64 bits lie between 2e-7 and 4.5e-7 of the 2-norm, and with a channel 10^6 times the others below 2e-6 of
+// each channel's.
 //
 // What bounds it. int8, 64 trees of up to 64 nodes over up to 4K tokens (16 heads, 8 of K/V, D 128, 55 GFLOP,
 // 298 MB): 167 us, 330 TFLOP/s; a 32-token tile takes the two wavefronts of a SIMD 1.6 us, nine
@@ -110,6 +113,17 @@ __device__ __forceinline__ void split2(float a, float x, float b, float y, uint3
   const f16x2 h = as_h2(hi);
   lo = as_u(f16x2{static_cast<_Float16>(__builtin_fmaf(a, x, -static_cast<float>(h[0]))),
                   static_cast<_Float16>(__builtin_fmaf(b, y, -static_cast<float>(h[1])))});
+}
+
+// The same with the low pieces 2^11 times as large: a low piece is up to 2^-12 of its high one, and so is not a subnormal
+// number before that is one.
+constexpr float kLoUp = 2048.f;
+__device__ __forceinline__ void split2_up(float a, float x, float b, float y, uint32_t& hi, uint32_t& lo) {
+  hi = as_u(f16x2{static_cast<_Float16>(__builtin_fmaf(a, x, -0.f)), static_cast<_Float16>(__builtin_fmaf(b, y, -0.f))});
+  asm("" : "+v"(hi));
+  const f16x2 h = as_h2(hi);
+  const float r0 = __builtin_fmaf(a, x, -static_cast<float>(h[0])), r1 = __builtin_fmaf(b, y, -static_cast<float>(h[1]));
+  lo = as_u(f16x2{static_cast<_Float16>(r0 * kLoUp), static_cast<_Float16>(r1 * kLoUp)});
 }
 
 // Byte J of two words, each a value + 128 -> the two values times 2^-9 in fp16, exact. A byte alone is that many
@@ -760,13 +774,17 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
 // ---- fp32 cache -----------------------------------------------------------------------------------
 
 // Trees of many rows: fp16 matrix instructions on K, V, q and weights in two fp16 pieces, three products
-// for each (the low pieces' own is below the last bit). A row of K, V or q is scaled by a power of two (K and q:
-// largest value in [2^10, 2^11), V: [2^4, 2^5)): an element keeps 22 bits down to 2^-13 (V: 2^-7) of its row's largest, and
-// 2^-35 (2^-29) of that below. All wavefronts take the same 32 tokens: each brings and splits a quarter of
+// for each (the low pieces' own is below the last bit). A row of K, V or q is scaled by a power of two (largest value in
+// [2^14, 2^15)), its low pieces by 2^11 more: an element keeps 22 bits down to 2^-29 of its row's largest, and is held to
+// 2^-51 of that below. (With the low pieces as they come and V in [2^4, 2^5), one channel 10^4 times the others left
+// those 8e-6; the scaling takes 1 us of 45.) The low pieces' products with q have sums of their own, those with the
+// weights take high pieces of 2^-11. All wavefronts take the same 32 tokens: each brings and splits a quarter of
 // them, two tokens and 8 dims a lane, into one half of LDS while the other is computed; V is laid down
 // with the tokens of a product step side by side, so that no wavefront transposes. Addresses in the loop are formed
 // anew for every tile: kept, they were spilled, and reading them back waits for the rows under way (57 us instead
 // of 47). Rows that are not finite leave NaN in the sums, and plain_rows takes over.
+constexpr int kPieceTop = 15;            // a row's largest value lies in [2^14, 2^15)
+constexpr float kVPieceUp = 1024.f;      // of that, what the weights do not take back (p v_scale lies near 2^kTop with V near 2^5)
 template <int D>
 __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a) {
   constexpr int KT = 32, KS = D / 32, DT = D / 16, kSide = KT * D * 2, kRowBytes = 4 * D, kHalf = 4 * kSide + 2 * KT * 4;
@@ -857,12 +875,12 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float each, down;
-      scale_of(kx[k], 11, each, down);
+      scale_of(kx[k], kPieceTop, each, down);
       u32x4 hi, lo;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h, l;
-        split2(kx[k][j / 2][j % 2 * 2], each, kx[k][j / 2][j % 2 * 2 + 1], each, h, l);
+        split2_up(kx[k][j / 2][j % 2 * 2], each, kx[k][j / 2][j % 2 * 2 + 1], each, h, l);
         hi[j] = h;
         lo[j] = l;
       }
@@ -870,13 +888,13 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
       *reinterpret_cast<u32x4*>(to + at) = hi;
       *reinterpret_cast<u32x4*>(to + kSide + at) = lo;
       if (chunk == 0) scales[row] = on[k] ? down : 0.f;
-      scale_of(vx[k], 5, up[k], down);
-      if (chunk == 0) scales[KT + row] = on[k] ? down : 0.f;
+      scale_of(vx[k], kPieceTop, up[k], down);
+      if (chunk == 0) scales[KT + row] = on[k] ? down * kVPieceUp : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {  // dim 8 chunk + j: row chunk of product j
       uint32_t h, l;
-      split2(vx[0][j / 4][j % 4], up[0], vx[1][j / 4][j % 4], up[1], h, l);
+      split2_up(vx[0][j / 4][j % 4], up[0], vx[1][j / 4][j % 4], up[1], h, l);
       const int at = (j * 16 + chunk) * 64 + 16 * ((place / 8) ^ (chunk / 4)) + place % 8 * 2;
       *reinterpret_cast<uint32_t*>(to + 2 * kSide + at) = h;
       *reinterpret_cast<uint32_t*>(to + 3 * kSide + at) = l;
@@ -927,7 +945,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
         top = max3_abs(top, x[c][ks][h][0], x[c][ks][h][1]);
         top = max3_abs(top, x[c][ks][h][2], x[c][ks][h][3]);
       }
-    const int e = 11 - max(__builtin_amdgcn_frexp_expf(max_over_fc(top)), -100);
+    const int e = kPieceTop - max(__builtin_amdgcn_frexp_expf(max_over_fc(top)), -100);
     // the sign of the softmax scale goes with q, so that the scores' order is the dots'; qs > 0: -inf * 0 below
     const float up = __builtin_copysignf(__builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23), a.scale);
     qs[c] = fmaxf(fabsf(a.scale) * kLog2e * __builtin_bit_cast(float, static_cast<uint32_t>(127 - e) << 23), 1e-37f);
@@ -937,7 +955,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h, l;
-        split2(x[c][ks][j / 2][j % 2 * 2], up, x[c][ks][j / 2][j % 2 * 2 + 1], up, h, l);
+        split2_up(x[c][ks][j / 2][j % 2 * 2], up, x[c][ks][j / 2][j % 2 * 2 + 1], up, h, l);
         hi[j] = h;
         lo[j] = l;
       }
@@ -958,34 +976,33 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
     const int lane = my_tid() % kWave, fr = lane % 16, fc = lane / 16;
     const float* const scales = reinterpret_cast<const float*>(tile + 4 * kSide);
     const uint32_t have = static_cast<uint32_t>(__ballot(scales[lane % KT] != 0.f));
-    f32x4 s[kCols][2] = {}, vv[2];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      f16x8 kh[2], kl[2];
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const char* p = tile + (16 * tt + fr) * 2 * D + 16 * ((4 * ks + fc) ^ fr);
-        kh[tt] = *reinterpret_cast<const f16x8*>(p);
-        kl[tt] = *reinterpret_cast<const f16x8*>(p + kSide);
-      }
-      // (four sums, so that a product does not wait for the one before)
-#pragma unroll
-      for (int g = 0; g < 3; ++g)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            s[c][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g == 0 ? kl[tt] : kh[tt], g == 1 ? ql[c][ks] : qh[c][ks], s[c][tt], 0, 0, 0);
-    }
+    f32x4 s[kCols][2], vv[2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
+      // (four sums, so that a product does not wait for the one before; the low pieces' in their own, kLoUp as large)
+      f32x4 high[kCols] = {}, low[kCols] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const char* p = tile + (16 * tt + fr) * 2 * D + 16 * ((4 * ks + fc) ^ fr);
+        const f16x8 kh = *reinterpret_cast<const f16x8*>(p), kl = *reinterpret_cast<const f16x8*>(p + kSide);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) low[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[c][ks], low[c], 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) high[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c][ks], high[c], 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) low[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c][ks], low[c], 0, 0, 0);
+      }
       const f32x4 kk = *reinterpret_cast<const f32x4*>(scales + 16 * tt + 4 * fc);
       vv[tt] = *reinterpret_cast<const f32x4*>(scales + KT + 16 * tt + 4 * fc);
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) s[c][tt] *= kk;
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[c][tt][e] = __builtin_fmaf(low[c][e], 1.f / kLoUp, high[c][e]) * kk[e];
     }
-    f16x8 ph[kCols], pl[kCols];
+    f16x8 ph[kCols], pl[kCols], pd[kCols];  // pd: for V's low pieces
     weights_of<DT>(s, vv, qs, see, ctx, base, have, o, ph, pl);
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) pd[c] = ph[c] * static_cast<_Float16>(1.f / kLoUp);
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += 2) {
       f16x8 vh[2], vl[2];
@@ -1001,7 +1018,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
         for (int d = 0; d < 2; ++d)
 #pragma unroll
           for (int c = 0; c < kCols; ++c)
-            o.acc[c][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g == 0 ? vl[d] : vh[d], g == 1 ? pl[c] : ph[c], o.acc[c][d0 + d], 0, 0, 0);
+            o.acc[c][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g == 0 ? vl[d] : vh[d], g == 0 ? pd[c] : g == 1 ? pl[c] : ph[c], o.acc[c][d0 + d], 0, 0, 0);
     }
   };
   // everyone's part of the next tile is there, and this one has been read; loads stay under way
@@ -1024,7 +1041,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a
     }
     meet();
   }
-  o.unscale = 1.f;
+  o.unscale = 1.f / kVPieceUp;
   float odd = 0.f;  // NaN where a sum is not finite
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {

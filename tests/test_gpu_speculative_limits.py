@@ -90,3 +90,45 @@ def test_the_race_does_not_see_a_shift(gpu, seqs, drawn, offset, temp):
     temps = [temp] * seqs
     got = b.verify(x, tokens, temps, u, noise, probs)
     assert check_walks(got, b.walks(x, tokens, np.full(seqs, temp, F32), u, noise, probs), NEAR) >= seqs - 4
+
+
+# ---- channels and trees of very different size --------------------------------------------------
+
+
+@pytest.mark.parametrize("hq", [2, 16])
+@pytest.mark.parametrize("v_size,k_size", [(1.0, 1.0), (1e4, 1.0), (1e6, 1.0), (1e8, 1.0), (1.0, 1e3), (1.0, 1e4), (1e6, 1e4)])
+def test_channels_of_very_different_size(gpu, hq, v_size, k_size):
+    """A float32 cache with one channel of V v_size times the others, one of K k_size times the others (its q as much
+    smaller) and one of q k_size times the others (its K as much smaller): every channel of the result by
+    itself is as near as with channels of one size, on the fp32 matrix instructions (few rows) and in fp16 pieces: a
+    float32 product's rounding is relative to each term, so that the bound on a result's 2-norm holds for a channel's."""
+    b = Batch(44, [333], [random_tree(np.random.default_rng(6), 24)], 16, gpu, heads=(hq, 2))
+    d = 128
+    (kc, vc), (k, v) = b.caches(d, "fp32")
+    q = b.rng.standard_normal((b.T, hq, d)).astype(F32)
+    v[..., 5] *= F32(v_size)
+    k[..., 9] *= F32(k_size)
+    q[..., 9] /= F32(k_size)
+    k[..., 77] /= F32(k_size)
+    q[..., 77] *= F32(k_size)
+    kc.copy_(torch.from_numpy(k))
+    vc.copy_(torch.from_numpy(v))
+    out = sp.tree_attention(b.put(q, F32), kc, vc, b.draft, d ** -0.5).cpu().numpy().astype(np.float64)
+    want = b.attend64(q, k, v, (None, None), d ** -0.5)
+    error = np.linalg.norm(out - want, axis=(0, 1)) / np.linalg.norm(want, axis=(0, 1))
+    assert (error <= 2e-6).all(), (error.argmax(), error.max())
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp32"])
+@pytest.mark.parametrize("nodes", [[64] + [1] * 30, [1, 2, 60, 64, 1, 3, 64, 50]])
+def test_large_trees_beside_small_ones(gpu, kind, nodes):
+    """Few rows on average with one large tree among them, and many with small ones among them: every tree by itself."""
+    rng = np.random.default_rng(len(nodes))
+    b = Batch(45, rng.integers(0, 700, len(nodes)).tolist(), [random_tree(rng, n) for n in nodes], 16, gpu, heads=(16, 2))
+    caches, (k, v) = b.caches(128, kind)
+    q = rng.standard_normal((b.T, 16, 128)).astype(F32)
+    out = sp.tree_attention(b.put(q, F32), *caches, b.draft, 0.09).cpu().numpy().astype(np.float64)
+    want = b.attend64(q, k, v, caches, 0.09)
+    for s in range(len(nodes)):
+        r = b.rows(s)
+        assert np.linalg.norm(out[r] - want[r]) <= 2e-6 * np.linalg.norm(want[r]), s
