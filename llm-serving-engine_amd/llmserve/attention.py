@@ -600,13 +600,16 @@ def paged_attention(
         return _attend(q, k_cache, v_cache, meta, scale)
     from .speculative import tree_attention
 
+    # the type that the batch has without trees: the native kernels' float32, else q's
+    native = meta.draft.native and (isinstance(k_cache, QuantizedKV) or k_cache.dtype == torch.float32)
+    dtype = torch.float32 if native else q.dtype
     if meta.rest is None:
-        return tree_attention(q, k_cache, v_cache, meta.draft, scale)
-    out = torch.empty_like(q, dtype=torch.float32)
+        return tree_attention(q, k_cache, v_cache, meta.draft, scale).to(dtype)
+    out = torch.empty_like(q, dtype=dtype)
     rows = meta.draft_rows
-    out.index_copy_(0, rows, tree_attention(q.index_select(0, rows), k_cache, v_cache, meta.draft, scale))
+    out.index_copy_(0, rows, tree_attention(q.index_select(0, rows), k_cache, v_cache, meta.draft, scale).to(dtype))
     rows = meta.rest_tokens
-    out.index_copy_(0, rows, _attend(q.index_select(0, rows), k_cache, v_cache, meta.rest, scale).float())
+    out.index_copy_(0, rows, _attend(q.index_select(0, rows), k_cache, v_cache, meta.rest, scale).to(dtype))
     return out
 
 

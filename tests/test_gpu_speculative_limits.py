@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from llmserve import speculative as sp
+from spec_steps import typed_step
 from spec_util import Batch, check_walks, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +133,20 @@ def test_large_trees_beside_small_ones(gpu, kind, nodes):
     for s in range(len(nodes)):
         r = b.rows(s)
         assert np.linalg.norm(out[r] - want[r]) <= 2e-6 * np.linalg.norm(want[r]), s
+
+
+# ---- types --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["int8", "fp32"])
+@pytest.mark.parametrize("long", [False, True])
+def test_a_batch_with_trees_has_the_type_it_has_without(gpu, dtype, kind, long):
+    """The kernels give float32 for every type of q, with trees and without."""
+    step = typed_step(dtype, kind, long, gpu, 64)
+    got, caches, meta = step(trees=True)
+    plain, *_ = step(trees=False)
+    assert got.dtype == plain.dtype == torch.float32 and got.shape == plain.shape
+    assert torch.equal(got[:5], sp.tree_attention(step.q[:5].contiguous(), *caches, meta.draft, 0.2))
+    assert long == (len(got) > 5)
+    assert (got[5:] - plain[5:]).norm() <= 2e-6 * plain[5:].norm()
