@@ -28,7 +28,7 @@ from .attention import AttentionMetadata, QuantizedKV, _model_placement, resolve
 from .kernels import load_fused_ops
 from .kv_cache import KVCache
 from .sampling import SampleRow
-from .speculative import commit_draft, verify
+from .speculative import check_requests, commit_draft, verify
 from .transformer import QuantCausalLM
 
 
@@ -98,11 +98,10 @@ class ModelRunner:
                 and len(logit_rows) == len(set(logit_rows)))
 
     def _collect(self, sched):
-        """The scheduled batch: copies its blocks; new token ids and positions end to end, lengths and
+        """The scheduled batch: new token ids and positions end to end, lengths and
         tables, the parents of the sequences whose drafted tokens form a tree (None: no such sequence;
         ``seq.spec_parents[i]`` is the index in ``seq.spec_tokens`` of the parent of draft ``i``, -1: the
         sequence's last token), and the index of every sequence's last new token."""
-        self.copy_blocks(getattr(sched, "block_copies", None) or [])
         ids: list[int] = []
         pos: list[int] = []
         q_lens, ctx_lens, tables, parents, last = [], [], [], [], []
@@ -129,11 +128,16 @@ class ModelRunner:
             last.append(len(ids) - 1)
         return ids, pos, q_lens, ctx_lens, tables, None if all(p is None for p in parents) else parents, last
 
-    def _forward_trees(self, ids, q_lens, ctx_lens, tables, parents):
+    def _copy_scheduled(self, sched) -> None:
+        """The batch's block copies: after its last check, so that a refused step leaves the cache as it was."""
+        self.copy_blocks(getattr(sched, "block_copies", None) or [])
+
+    def _forward_trees(self, sched, ids, q_lens, ctx_lens, tables, parents):
         """(metadata, hidden states) of a batch with trees of drafted tokens."""
         cfg, dev = self.model.cfg, self.device
         meta = AttentionMetadata.build(q_lens, ctx_lens, tables, self.block_size, dev, self.attention_backend,
                                        parents, (cfg.num_attention_heads, cfg.num_key_value_heads))
+        self._copy_scheduled(sched)
         return meta, self.model(torch.tensor(ids, dtype=torch.long, device=dev), meta.positions,
                                 self.cache.layers, meta)
 
@@ -145,7 +149,8 @@ class ModelRunner:
         ``speculative.verify`` accepts under ``rows[i]`` and moves their cache rows behind the computed
         ones. Returns the new tokens of each sequence, accepted drafts first: with ``k`` of them the
         sequence has ``k`` more computed tokens, the last of the ``k`` not among them.
-        ``draft_probs`` [new tokens, vocabulary]: as ``speculative.verify_draft``."""
+        ``draft_probs`` [new tokens, vocabulary]: as ``speculative.verify_draft``. What ``verify`` refuses is
+        refused before anything is copied or written."""
         ids, _, q_lens, ctx_lens, tables, parents, _ = self._collect(sched)
         if len(rows) != len(q_lens):
             raise ValueError("one SampleRow per scheduled sequence")
@@ -154,13 +159,19 @@ class ModelRunner:
             if item.num_new_tokens != 1 + len(getattr(seq, "spec_tokens", None) or []) or (
                     len(seq.token_ids()) != seq.num_computed_tokens + 1):
                 raise ValueError("a verified sequence has one uncomputed token, and its drafts are all scheduled")
-        if not q_lens:
-            return []
+        check_requests(rows)
+        vocab = self.model.cfg.vocab_size
+        if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.shape != (len(ids), vocab)
+                                        or draft_probs.device != self.device):
+            raise ValueError(f"draft_probs must be a float32 {[len(ids), vocab]} tensor on {self.device}")
         self._check_tables(tables, ctx_lens)
-        self._check_ids(ids, self.model.cfg.vocab_size)
+        self._check_ids(ids, vocab)
+        if not q_lens:
+            self._copy_scheduled(sched)
+            return []
         chains = [list(range(-1, n - 1)) for n in q_lens]
         parents = chains if parents is None else [c if p is None else p for p, c in zip(parents, chains)]
-        meta, hidden = self._forward_trees(ids, q_lens, ctx_lens, tables, parents)
+        meta, hidden = self._forward_trees(sched, ids, q_lens, ctx_lens, tables, parents)
         logits = self.model.compute_logits(hidden).float()
         tokens = torch.tensor(ids, dtype=torch.long, device=logits.device)
         got = verify(logits, meta.draft, tokens, rows, q_lens, draft_probs)
@@ -186,11 +197,12 @@ class ModelRunner:
         m = self.model
         self._check_ids(ids, m.cfg.vocab_size)
         if parents is not None:
-            meta, hidden = self._forward_trees(ids, q_lens, ctx_lens, tables, parents)
+            meta, hidden = self._forward_trees(sched, ids, q_lens, ctx_lens, tables, parents)
             if not rows:
                 return torch.empty(0, m.cfg.vocab_size)
             sel = torch.tensor(rows, dtype=torch.long, device=self.device)
             return m.compute_logits(hidden.index_select(0, sel)).float().cpu()
+        self._copy_scheduled(sched)
         # The forward always runs, also when no row is sampled: a step made only of non-final
         # prompt chunks (chunked prefill) writes its K/V here and samples nothing.
         if self._decode_step_ok(q_lens, rows):

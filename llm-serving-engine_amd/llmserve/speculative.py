@@ -188,6 +188,13 @@ def commit_draft(cache, draft: DraftBatch, verified: Verified) -> None:
         ops.commit_draft_(data, scales, draft.plan, path, accepted, draft.block_tables, draft.block_size)
 
 
+def check_requests(rows: list[SampleRow]) -> None:
+    """Refuses requests that ``verify`` cannot serve."""
+    for r in rows:
+        if _penalized(r.params) or r.allowed_token_ids is not None or r.banned_token_ids:
+            raise ValueError("penalties and allowed / banned tokens are not supported with drafted tokens")
+
+
 def verify(logits: torch.Tensor, draft: DraftBatch, draft_tokens: torch.Tensor, rows: list[SampleRow],
            nodes: list[int], draft_probs: torch.Tensor | None = None) -> Verified:
     """``verify_draft`` for requests: ``rows[s]`` the sampling parameters and generator of sequence ``s``,
@@ -197,9 +204,7 @@ def verify(logits: torch.Tensor, draft: DraftBatch, draft_tokens: torch.Tensor, 
     emitted, are refused."""
     if len(rows) != draft.sequences or len(nodes) != len(rows) or sum(nodes) != logits.shape[0]:
         raise ValueError("one row and one node count per sequence")
-    for r in rows:
-        if _penalized(r.params) or r.allowed_token_ids is not None or r.banned_token_ids:
-            raise ValueError("penalties and allowed / banned tokens are not supported with drafted tokens")
+    check_requests(rows)
     dev, v = logits.device, logits.shape[1]
     uniforms, noise, temps, at = [], [], [], 0
     cut = logits
@@ -367,5 +372,5 @@ def _commit_torch(tensors, draft: DraftBatch, path: torch.Tensor, accepted: torc
                     t[dst] = t[src]
 
 
-__all__ = ["MAX_NODES", "DraftBatch", "Verified", "commit_draft", "draft_batch", "tree_attention", "verify",
+__all__ = ["MAX_NODES", "DraftBatch", "Verified", "check_requests", "commit_draft", "draft_batch", "tree_attention", "verify",
            "verify_draft"]

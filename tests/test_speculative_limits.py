@@ -2,9 +2,13 @@
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
+from llmserve.model_runner import ModelRunner
+from llmserve.sampling import SampleRow, SamplingParams
 from llmserve.speculative import tree_attention
 from spec_steps import typed_step
 
@@ -30,3 +34,50 @@ def test_trees_in_16_bits_over_other_caches(dtype, kind):
     got, caches, meta = step(trees=True)
     assert got.dtype == dtype
     assert torch.equal(got, tree_attention(step.q.float(), *caches, meta.draft, 0.2).to(dtype))
+
+
+def test_a_refused_step_leaves_the_cache_as_it_was():
+    """Requests, probabilities, tables, ids and trees that are refused: before a block is copied or the model runs."""
+    copied = []
+
+    class Model:
+        cfg = SimpleNamespace(vocab_size=50, num_attention_heads=4, num_key_value_heads=2)
+
+        def __call__(self, *args):
+            raise LookupError("the model runs")
+
+    runner = ModelRunner.__new__(ModelRunner)
+    runner.cache, runner.block_size, runner.model = SimpleNamespace(layers=[], num_blocks=4), 16, Model()
+    runner.device, runner.attention_backend = torch.device("cpu"), "torch"
+    runner.copy_blocks = copied.append
+
+    def sched(drafts=(8, 9, 3), up=(-1, -1, 0), table=(0,), known=(5, 6, 7)):
+        seq = SimpleNamespace(token_ids=lambda: list(known), num_computed_tokens=2, spec_tokens=list(drafts),
+                              spec_parents=None if up is None else list(up), block_table=list(table))
+        item = SimpleNamespace(seq=seq, num_new_tokens=len(known) - 2 + len(drafts))
+        return SimpleNamespace(scheduled=[item], block_copies=[(1, 2)])
+
+    def row(**kw):
+        return SampleRow(SamplingParams(**{k: v for k, v in kw.items() if k != "banned"}), [], [], None,
+                         **({"banned_token_ids": kw["banned"]} if "banned" in kw else {}))
+
+    ok = row()
+    for rows, kw in (([row(presence_penalty=1.0)], {}), ([row(repetition_penalty=1.1)], {}), ([row(banned=[3])], {}), ([], {}),
+                     ([ok], dict(draft_probs=torch.ones(4, 49))), ([ok], dict(draft_probs=torch.ones(4, 50).double()))):
+        with pytest.raises(ValueError):
+            runner.verify_step(sched(), rows, **kw)
+    chain = [1] * 64
+    for bad, error in ((sched(table=(9,)), IndexError), (sched(drafts=(8, 9, 50)), IndexError), (sched(up=(-1, 1, 0)), ValueError),
+                       (sched(up=(-1, -1)), ValueError), (sched(known=(5, 6)), ValueError),
+                       (sched(chain, None, (0, 1, 2, 3, 0)), ValueError), (sched(table=()), ValueError)):
+        with pytest.raises(error):
+            runner.verify_step(bad, [ok])
+        if bad.scheduled[0].seq.spec_parents is not None and len(bad.scheduled[0].seq.token_ids()) > 2:
+            with pytest.raises(error):
+                runner.execute(bad, [0])
+    assert copied == []
+    for run in (lambda: runner.verify_step(sched(), [ok]), lambda: runner.execute(sched(), [0])):
+        with pytest.raises(LookupError):
+            run()
+    assert copied == [[(1, 2)], [(1, 2)]]
+    assert runner.verify_step(SimpleNamespace(scheduled=[], block_copies=[(0, 3)]), []) == [] and copied[2] == [(0, 3)]
