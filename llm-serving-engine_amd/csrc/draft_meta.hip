@@ -228,6 +228,15 @@ __global__ __launch_bounds__(kThreads) void draft_metadata_kernel(MetaArgs a) {
   none(d.first + d.nodes, s + 1 < a.S ? tree_of(a, s + 1).first : a.T);
 }
 
+// A batch without sequences: all of its rows belong to no tree.
+__global__ __launch_bounds__(kThreads) void no_trees_kernel(int64_t T, int64_t* positions, int64_t* slots, int64_t* ancestors) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (t >= T) return;
+  positions[t] = 0;
+  slots[t] = -1;
+  ancestors[t] = 0;
+}
+
 }  // namespace
 
 extern "C" int64_t llmserve_draft_plan_items(int64_t S, int64_t T, int64_t max_blocks, int64_t block_size,
@@ -253,7 +262,14 @@ extern "C" int llmserve_draft_metadata(const int64_t* context_lens, const int64_
   LSH_CHECK(S >= 0 && T >= 0 && max_blocks >= 0 && block_size >= 1 && G >= 1 && Hk >= 1,
             "draft_metadata: bad sizes (S=%lld, T=%lld, max_blocks=%lld, block_size=%lld, G=%lld, Hk=%lld)",
             (long long)S, (long long)T, (long long)max_blocks, (long long)block_size, (long long)G, (long long)Hk);
-  if (S == 0) return LLMSERVE_OK;
+  if (S == 0 && T == 0) return LLMSERVE_OK;
+  if (S == 0) {
+    LSH_CHECK(T < (1LL << 24), "draft_metadata: batch or context too large");
+    LSH_CHECK(positions && slots && ancestors, "draft_metadata: null pointer");
+    lsh::launch(no_trees_kernel, dim3(static_cast<unsigned>((T + kThreads - 1) / kThreads)), dim3(kThreads), 0, lsh::as_stream(stream),
+                true, T, positions, slots, ancestors);
+    return lsh::launch_status("draft_metadata");
+  }
   LSH_CHECK(max_blocks >= 1, "draft_metadata: sequences without blocks");
   LSH_CHECK(S <= (1 << 16) && T < (1LL << 24) && max_blocks < (1LL << 30) && block_size < (1LL << 30) &&
                 max_blocks * block_size < (1LL << 30) && G <= 1024 && Hk <= 4096,

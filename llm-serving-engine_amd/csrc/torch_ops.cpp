@@ -973,7 +973,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> draft_metadata(
   const int64_t items = llmserve_draft_plan_items(S, T, block_tables.size(1), block_size, G, kv_heads);
   auto nodes = at::empty({3, T}, context_lens.options());
   auto plan = at::empty({llmserve_draft_plan_bytes(S, T, items, kv_heads)}, context_lens.options().dtype(at::kByte));
-  if (S == 0) nodes.fill_(-1);
   int64_t* p = nodes.data_ptr<int64_t>();
   check_status(llmserve_draft_metadata(
       context_lens.data_ptr<int64_t>(), draft_start.data_ptr<int64_t>(), parents.data_ptr<int64_t>(),

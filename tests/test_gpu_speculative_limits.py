@@ -150,3 +150,15 @@ def test_a_batch_with_trees_has_the_type_it_has_without(gpu, dtype, kind, long):
     assert torch.equal(got[:5], sp.tree_attention(step.q[:5].contiguous(), *caches, meta.draft, 0.2))
     assert long == (len(got) > 5)
     assert (got[5:] - plain[5:]).norm() <= 2e-6 * plain[5:].norm()
+
+
+# ---- a batch without sequences --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 7, 1000])
+def test_rows_without_sequences(gpu, rows):
+    put = lambda x: torch.tensor(x, dtype=torch.long, device=gpu)  # noqa: E731
+    tables = torch.empty(0, 3, dtype=torch.long, device=gpu)
+    d = sp.draft_batch(put([]), put([0]), put([-1] * rows), tables, 16, 2, 1)
+    assert d.native and len(d.positions) == len(d.slots) == len(d.ancestors) == rows
+    assert bool((d.positions == 0).all()) and bool((d.slots == -1).all()) and bool((d.ancestors == 0).all())

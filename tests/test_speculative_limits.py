@@ -7,9 +7,10 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from llmserve._native import capi
 from llmserve.model_runner import ModelRunner
 from llmserve.sampling import SampleRow, SamplingParams
-from llmserve.speculative import tree_attention
+from llmserve.speculative import draft_batch, tree_attention
 from spec_steps import typed_step
 
 
@@ -81,3 +82,12 @@ def test_a_refused_step_leaves_the_cache_as_it_was():
             run()
     assert copied == [[(1, 2)], [(1, 2)]]
     assert runner.verify_step(SimpleNamespace(scheduled=[], block_copies=[(0, 3)]), []) == [] and copied[2] == [(0, 3)]
+
+
+def test_rows_without_sequences():
+    empty = torch.empty(0, dtype=torch.long)
+    d = draft_batch(empty, torch.zeros(1, dtype=torch.long), torch.tensor([-1] * 7), torch.empty(0, 3, dtype=torch.long), 16, 2, 1)
+    assert d.positions.tolist() == d.ancestors.tolist() == [0] * 7 and d.slots.tolist() == [-1] * 7
+    f = capi().llmserve_draft_metadata
+    assert f(*[None] * 4, 0, 7, 3, 16, 1, 1, *[None] * 4, 0, None) == 1
+    assert "null pointer" in capi().llmserve_last_error().decode()
