@@ -13,7 +13,7 @@
 // One wavefront per sequence, a lane per node: the masks close in six doublings
 // (mask |= mask[to], to = to[to]), all in registers. Every workgroup derives the work plan of the
 // attention (draft.h) from all lengths by itself, so that no workgroup waits for another. Bound by its chain
-// of dependent loads, sums and divisions: 7.6 us for one sequence, 9.4 for 128; the call takes 9.4, most of it on the host.
+// of dependent loads, sums and divisions: 7.7 us for one sequence, 9.6 for 128; the call takes 9.6, most of it on the host.
 #include "draft.h"
 
 namespace {

@@ -31,9 +31,9 @@
 // before, from its slices, and reads a slice of the node it comes to. Deeper nodes, and drawn drafts, whose
 // residuals are sums over rows, are left to the walk, whose workgroup reads each row when it gets there.
 // 24 trees of up to 64 nodes with 152K tokens, paths of up to 6: a launch takes
-// 6 us, 57 us in all; with every row read by the walk's own workgroup (12 us a row, its CU's exponentials) it was 89.
-// One stream of 5 nodes: 16.6 us, three launches from the host; 32 chains with their drafter's distributions: 42 us, 2.1 TB/s
-// (rows 16, race 13).
+// 6 us, 61 to 71 us in all; with every row read by the walk's own workgroup (12 us a row, its CU's exponentials) it was 89.
+// One stream of 5 nodes: 15.5 us, three launches from the host; 32 chains with their drafter's distributions: 41 us, 2.1 TB/s
+// (rows 16, walks 10, race 14).
 #include <algorithm>
 
 #include "draft.h"
@@ -50,11 +50,12 @@ constexpr int kPer = 4;                 // its 16-byte loads for each thread
 constexpr int kSlice = kSliceThreads * kPer * 4;  // tokens of a slice
 constexpr int kWalkWaves = 16;          // of the workgroup of a walk that reads rows itself
 // Logits up to which the rows' softmaxes are formed ahead of the walks: of drawn drafts, and of given ones (trees of up to
-// 58 nodes, 98511 tokens: 52 M 38 us against 53 with a launch a level, 71 M 44 against 50, 88 M 79 against 56).
+// 58 nodes, 98511 tokens, paths of up to 8: 47 M 41 us against 52 with a launch a level, 62 M 50 against 60, 77 M 56 against 57;
+// what a launch a level takes hardly grows).
 constexpr int64_t kAhead = 150LL << 20;
 constexpr int64_t kAheadGiven = 75LL << 20;
 // Workgroups of the race up to which each of them walks by itself instead of a launch before: 38 (one stream of 152K
-// tokens) 15.8 us against 18.5, 988 27.8 against 34.0, 2432 49.8 against 52.0, 4864 90 against 87.
+// tokens) 17.5 us against 21.4, 988 34.5 against 40.1, 2432 62.7 against 61.8, 4864 68.6 against 60.6.
 constexpr int64_t kFused = 3000;
 // Nodes of a path that have their own launch: one that no path comes to takes 2 us, a row left to the walk 12.
 constexpr int kLevels = 12;

@@ -25,14 +25,14 @@
 // Errors against 64 bits lie between 2e-7 and 4.5e-7 of the 2-norm, and with a channel 10^6 times the others below 2e-6 of
 // each channel's.
 //
-// What bounds it. int8, 64 trees of up to 64 nodes over up to 4K tokens (16 heads, 8 of K/V, D 128, 55 GFLOP,
-// 298 MB): 167 us, 330 TFLOP/s; a 32-token tile takes the two wavefronts of a SIMD 1.6 us, nine
-// tenths of it the issue of vector instructions (13 for each score of a lane, 80 to widen V), the products hidden
-// behind them. 16 trees of 26 nodes: 46 us, 1.9 TB/s: 22 us of tiles, the rest the starts and ends of the workgroups (plan,
-// table, q: 8 us, joining 4 us) and the second launch. One stream: 15 us, two launches and one tile. Single tokens of 64
-// sequences over 2K tokens: 97 us, 3.5 TB/s. fp32: 32 sequences of 5 nodes (10
-// rows) read 4.7 TB/s; 208 rows a kv head take 47 us (92 TFLOP/s) in fp16 pieces, 81 on the fp32 matrix instructions, which
-// were busy for half of that time; 52 rows 104 us and 3.0 TB/s in pieces, 122 without.
+// What bounds it. int8, 32 trees of up to 64 nodes over 1K to 8K tokens (1716 nodes, 16 heads, 8 of K/V, D 128, 55 GFLOP,
+// 298 MB): 166 us, 330 TFLOP/s; vector instructions (13 for each score of a lane, 80 to widen V) are issued in 64 % of the
+// SIMDs' cycles, the matrix unit is busy in 31 %, hidden behind them. 16 trees of 26 nodes: 46 us, 1.9 TB/s: 22 us
+// of tiles, the rest the starts and ends of the workgroups (plan, table, q: 8 us, joining 4 us) and the second launch
+// (61 % and 22 %). One stream: 16 us of kernels, two launches and one tile. Single tokens of 64
+// sequences over 2K tokens: 78 us, 3.5 TB/s. fp32: 32 sequences of 5 nodes (10 rows) over 1K to 4K tokens 136 us, 4.9 TB/s; 208
+// rows a kv head 46 us (95 TFLOP/s) in fp16 pieces, vector instructions in 49 %, products in 18 % of the cycles. D 64, 16
+// trees of 26 nodes over 512 to 4K tokens, 8 kv heads: int8 29 us, 1.5 TB/s, fp32 46 us, 3.5 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -1376,8 +1376,10 @@ __global__ __launch_bounds__(kWave) void tree_row_kernel(TreeArgs a) {
 template <typename E, int D>
 auto tiled_kernel(const TreeArgs& a) {
   if constexpr (std::is_same_v<E, float>) {
-    // fp16 pieces where trees have more than 32 rows a kv head on average (208: 47 us against 81; 52: 104 against 122; 10: 168
-    // against 142: with up to 32 rows three wavefronts only stage)
+    // fp16 pieces where trees have more than 32 rows a kv head on average (208: 49 us against 83; 52: 106 against 120; 40: 114
+    // against 127; 10: 169 against 136: with up to 32 rows three wavefronts only stage). Of trees that differ much the
+    // average says less: one of 64 nodes among 31 single tokens takes 192 us, 137 in pieces; one single token among 7 trees 61
+    // in pieces, 102 without.
     if constexpr (D == 128)
       if (a.T * a.G > kSplitRows * a.S) return tree_split_kernel<D>;
     return tree_f32_kernel<D>;

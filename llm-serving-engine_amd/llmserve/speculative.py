@@ -17,7 +17,8 @@ its block table and rotated for position ``c + depth``. One step:
 
 On a ROCm device these are HIP kernels (``llmserve_draft_metadata``, ``llmserve_paged_attention_tree``,
 ``llmserve_verify_draft``, ``llmserve_commit_draft``) on the current stream without synchronization,
-so a step can be captured into a graph; elsewhere, or without the native library, torch ops.
+so a step of these four can be captured into a graph; elsewhere, or without the native library, torch ops.
+``verify`` draws its numbers request by request and copies parameters from the host: it is not for a graph.
 """
 
 from __future__ import annotations
@@ -83,8 +84,9 @@ def draft_batch(context_lens: torch.Tensor, draft_start: torch.Tensor, parents: 
     """The trees of one step. ``context_lens`` [S]: cached tokens of each sequence, without its tree;
     ``draft_start`` [S + 1]: where each tree begins in the flat stream, and the end of the last;
     ``parents`` [T]; ``block_tables`` [S, max_blocks]: blocks of the cached tokens and the nodes; all
-    int64 on one device. ``max_nodes`` bounds the nodes of a tree (at most 64), ``max_depth`` the drafts
-    of a path (``max_nodes - 1`` when not given). The values are read on the device: a parent that is no
+    int64 on one device. ``max_depth`` is the most drafts of a path: a walk ends there. ``max_nodes`` (at most 64)
+    is the largest tree that the caller has, and gives ``max_depth`` when that is not given (``max_nodes - 1``);
+    trees are taken as they come, up to 64 nodes, whatever it says. The values are read on the device: a parent that is no
     earlier node makes a root, and rows of no tree (past a tree's 64th node, outside
     ``draft_start``) get slot -1 and are left alone by the step's kernels. ``native=False``: torch ops
     for the whole step, also on a ROCm device."""
@@ -115,7 +117,7 @@ def tree_attention(q: torch.Tensor, k_cache, v_cache, draft: DraftBatch, scale: 
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the nodes (q [T, Hq, D]) over a layer's caches, which hold the nodes' K/V already
     (``draft.slots``): ``QuantizedKV`` pairs (key smoothing as ``paged_attention`` applies it) or float32
-    tensors [slots, Hk, D]. Rows of no tree keep what ``out`` holds (they are undefined when it is not given);
+    tensors [slots, Hk, D]; float32 for every type of q. Rows of no tree keep what ``out`` holds (they are undefined when it is not given);
     ``out`` must not share memory with ``q``."""
     quantized = isinstance(k_cache, QuantizedKV)
     if quantized != isinstance(v_cache, QuantizedKV):
