@@ -6,6 +6,8 @@ Tolerances are those of ``test_gpu_speculative.py`` unless a test derives its ow
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -162,3 +164,50 @@ def test_rows_without_sequences(gpu, rows):
     d = sp.draft_batch(put([]), put([0]), put([-1] * rows), tables, 16, 2, 1)
     assert d.native and len(d.positions) == len(d.slots) == len(d.ancestors) == rows
     assert bool((d.positions == 0).all()) and bool((d.slots == -1).all()) and bool((d.ancestors == 0).all())
+
+
+def test_a_step_without_sequences(gpu):
+    """Attention leaves every row alone, verification and commit have nothing to do."""
+    put = lambda x: torch.tensor(x, dtype=torch.long, device=gpu)  # noqa: E731
+    d = sp.draft_batch(put([]), put([0]), put([-1] * 5), torch.empty(0, 3, dtype=torch.long, device=gpu), 16, 4, 2)
+    kc, vc = (torch.randn(48, 2, 128, device=gpu) for _ in range(2))
+    before = kc.clone()
+    q = torch.randn(5, 4, 128, device=gpu)
+    out = sp.tree_attention(q, kc, vc, d, 0.1, out=torch.full_like(q, -7.5))
+    assert bool((out == -7.5).all())
+    got = sp.verify_draft(torch.randn(5, 11, device=gpu), d, put([0] * 5), torch.empty(0, device=gpu), torch.rand(5, device=gpu),
+                          torch.empty(0, 11, device=gpu))
+    assert got.accepted.shape == (0,) and got.path.shape == got.tokens.shape == (0, 64)
+    sp.commit_draft(SimpleNamespace(layers=[(kc, vc)]), d, got)
+    assert torch.equal(kc, before)
+
+
+def test_sums_over_a_row_in_a_graph(gpu):
+    """Rows whose rest is summed, captured and replayed with other rows between eager calls: every replay the eager result."""
+    v, seqs = 4099, 12
+    b = Batch(46, [2] * seqs, [[-1, 0, 0]] * seqs, 16, gpu)
+    rng = np.random.default_rng(46)
+    sets = []
+    for i in range(3):
+        x = np.full((b.T, v), -np.inf, F32)
+        tokens = np.zeros(b.T, np.int64)
+        for s in range(seqs):
+            pair = rng.choice(v, 2, replace=False)
+            x[3 * s, pair] = [0.0, -13.31 - rng.random()]
+            x[3 * s + 1: 3 * s + 3, rng.integers(v)] = 1.0
+            tokens[3 * s + 1: 3 * s + 3] = pair
+        sets.append((b.put(x, F32), b.put(tokens)))
+    x, tokens = (t.clone() for t in sets[0])
+    numbers = [torch.ones(seqs, device=gpu), b.put([UNDER_ONE] * b.T, F32), b.put(rng.exponential(size=(seqs, v)), F32)]
+    eager = [sp.verify_draft(y, b.draft, t, *numbers) for y, t in sets]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sp.verify_draft(x, b.draft, tokens, *numbers)
+    for i in (1, 0, 2, 1):
+        x.copy_(sets[i][0])
+        tokens.copy_(sets[i][1])
+        graph.replay()
+        assert bool((got.accepted == 1).all())
+        for a, w in ((got.accepted, eager[i].accepted), (got.path, eager[i].path), (got.tokens, eager[i].tokens)):
+            assert torch.equal(a, w)
+        sp.verify_draft(x, b.draft, tokens, *numbers)

@@ -10,7 +10,7 @@ import torch
 from llmserve._native import capi
 from llmserve.model_runner import ModelRunner
 from llmserve.sampling import SampleRow, SamplingParams
-from llmserve.speculative import draft_batch, tree_attention
+from llmserve.speculative import draft_batch, tree_attention, verify_draft
 from spec_steps import typed_step
 
 
@@ -91,3 +91,14 @@ def test_rows_without_sequences():
     f = capi().llmserve_draft_metadata
     assert f(*[None] * 4, 0, 7, 3, 16, 1, 1, *[None] * 4, 0, None) == 1
     assert "null pointer" in capi().llmserve_last_error().decode()
+
+
+def test_trees_larger_than_max_nodes_are_taken():
+    """``max_nodes`` gives the depth limit only: a larger tree is whole, its path ends at the limit."""
+    one = torch.zeros(1, dtype=torch.long)
+    d = draft_batch(one, torch.tensor([0, 4]), torch.tensor([-1, 0, 1, 2]), one[None], 16, 2, 1, max_nodes=2)
+    assert d.max_depth == 1 and d.ancestors.tolist() == [1, 3, 7, 15] and d.slots.tolist() == [0, 1, 2, 3]
+    x = torch.zeros(4, 5)
+    x[:, 3] = 9
+    got = verify_draft(x, d, torch.tensor([0, 3, 3, 3]), torch.zeros(1), torch.zeros(4), torch.ones(1, 5))
+    assert got.path.tolist() == [[0, 1]] and got.tokens.tolist() == [[3, 3]]
