@@ -115,8 +115,8 @@ __device__ __forceinline__ void split2(float a, float x, float b, float y, uint3
                   static_cast<_Float16>(__builtin_fmaf(b, y, -static_cast<float>(h[1])))});
 }
 
-// The same with the low pieces 2^11 times as large: a low piece is up to 2^-12 of its high one, and so is not a subnormal
-// number before that is one.
+// The same with the low pieces 2^11 times as large (a low piece is up to 2^-12 of its high one): rounded to their smallest
+// step, 2^-24, they are off by 2^-36, which is 2^-22 of the smallest high piece that is a normal number.
 constexpr float kLoUp = 2048.f;
 __device__ __forceinline__ void split2_up(float a, float x, float b, float y, uint32_t& hi, uint32_t& lo) {
   hi = as_u(f16x2{static_cast<_Float16>(__builtin_fmaf(a, x, -0.f)), static_cast<_Float16>(__builtin_fmaf(b, y, -0.f))});
