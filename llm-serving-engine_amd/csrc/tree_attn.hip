@@ -16,13 +16,13 @@
 // being any four groups of the row's), V's is done by byte permutes in registers (int8) or is none
 // at all (fp32: one register is one element). A row's running reference and sum are per-lane scalars.
 //
-// Precision. int8: the scores are exact integer products of the codes with q in three signed digits: an element of
-// q' is held to 2^-24 of its row's largest one, and a score to that times the sum of its token's |code| (less than
-// fp32 keeps where the largest elements of q' meet codes near 0 only). Codes of V are exact in fp16, the weights two
-// fp16 pieces after scaling by a power of two (22 bits); scales stay in fp32 on the score and the weight. fp32: fp32
+// Precision is fp32's. int8: the scores are exact integer products of the codes with q in three signed digits (23 bits of
+// the row's largest element), or where few elements come near that one, of codes in fp16 with q in two fp16 pieces. Codes
+// of V are exact in fp16, the weights two fp16 pieces after scaling by a power of two (22 bits); scales stay in fp32 on
+// the score and the weight. fp32: fp32
 // matrix instructions (a step's sums formed apart and added once), for a head size of 128 and more than 32 rows a
 // tree on average fp16 ones on two pieces of everything: 22 bits of every element down to 2^-29 of its row's largest.
-// Errors against 64 bits lie between 2e-7 and 4.5e-7 of the 2-norm, and with a channel 10^6 times the others below 2e-6 of
+// Errors against 64 bits lie between 2e-7 and 4.5e-7 of the 2-norm, and with channels of very different size below 2e-6 of
 // each channel's.
 //
 // What bounds it. int8, 32 trees of up to 64 nodes over 1K to 8K tokens (1716 nodes, 16 heads, 8 of K/V, D 128, 55 GFLOP,
@@ -135,6 +135,13 @@ __device__ __forceinline__ uint32_t bytes_to_h2(uint32_t x0, uint32_t x1) {
   return as_u(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(x1, x0, 0x0c040c00u + 0x10001u * J)), up, zero));
 }
 constexpr float kVUp = 512.f;
+// Four int8 codes of a word, in order, as two words of fp16, times 2^-9.
+__device__ __forceinline__ u32x2 codes_to_h2(uint32_t codes) {
+  const f16x2 up = {32768, 32768}, zero = {-0.25, -0.25};
+  const uint32_t x = codes ^ 0x80808080u;
+  return u32x2{as_u(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(x, x, 0x0c010c00u)), up, zero)),
+               as_u(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(x, x, 0x0c030c02u)), up, zero))};
+}
 
 // What a wavefront of a workgroup computes.
 struct Work {
@@ -449,6 +456,11 @@ __device__ __forceinline__ void finish(const TreeArgs& a, const Work& w, Rows<D 
 // the other. K's 16-byte pieces are permuted within a row, so that 16 tokens' pieces lie in different banks.
 // The scores are int8 products: q is scaled to integers of 23 bits, in three signed digits of 8, whose
 // products with the codes are summed exactly in 32 bits (K needs no widening). V is widened to fp16.
+// An element of q is so held to 2^-24 of its row's largest one: where K's codes in the large channels are near 0, that is what
+// a score has left (a channel of q 100 times the others, its K as much smaller: 3e-6 of the result, 1000: 4e-5). A workgroup
+// with a row of such elements (kEven) therefore takes q in two fp16 pieces (22 bits of an element down to 2^-29 of the
+// largest) and widens K too: 58 us instead of 49 for 16 trees of 26 nodes, 193 instead of 168 for the largest. The test for it
+// takes no time that shows.
 template <int D>
 struct Tile8 {
   static constexpr int KT = 32;
@@ -457,6 +469,71 @@ struct Tile8 {
   static constexpr int kLoads = kSide / 1024;         // 1 KB loads of K, or V
   static constexpr int kChunks = D / 16;              // 16-byte pieces of a row
 };
+// q as the score products take it.
+template <int D>
+struct Digits {
+  u32x4 d[kCols][D / 64][3];  // the largest last
+};
+template <int D>
+struct Pieces {
+  f16x8 hi[kCols][D / 64][2], lo[kCols][D / 64][2];  // lo: times kLoUp
+};
+// A row takes pieces whose elements' exponents are less than its largest one's by more than this on the mean (normally
+// distributed ones' by 2.4, with one of them 16 times as large by 5; an element of 0 counts as one of 1).
+constexpr float kEven = 4.5f;
+constexpr int kPieceTop = 15;  // a row in pieces has its largest value in [2^14, 2^15)
+
+// A wavefront's rows in pieces: lane (fr, fc) dims fc D / 4 .. + D / 4 of row fr. `qs`: as for digits, for codes times 2^-9.
+template <int D>
+__device__ __forceinline__ Pieces<D> pieces_of(const TreeArgs& a, const Work& w, int lane, float (&qs)[kCols]) {
+  const int fr = lane % 16, fc = lane / 16;
+  Pieces<D> q;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    const int row = w.row0 + min(kWaveRows * w.rw + 16 * c + fr, w.rows - 1);
+    const int node = row / a.G, head = w.kvh * a.G + row % a.G;
+    const float* qp = a.q + (static_cast<int64_t>(w.first + node) * a.Hq + head) * D + fc * (D / 4);
+    const float* mp = a.q_mult + static_cast<int64_t>(head) * D + fc * (D / 4);
+    f32x4 x[D / 16];
+    float top = 0.f, odd = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      x[i] = *reinterpret_cast<const f32x4*>(qp + 4 * i);
+      if (a.q_mult) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(mp + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = __fmul_rn(x[i][e], y[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        top = fmaxf(top, fabsf(x[i][e]));
+        odd = __builtin_fmaf(x[i][e], 0.f, odd);
+      }
+    }
+    const int e = kPieceTop - max(__builtin_amdgcn_frexp_expf(max_over_fc(top)), -100);
+    const float up = __builtin_copysignf(__builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23), a.scale);
+    const float down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - e) << 23);
+    qs[c] = fmaxf(fabsf(a.scale) * kLog2e * kVUp * down, 1e-37f) + sum_over_fc(odd);
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 y = x[4 * s + 2 * h + j / 2];
+          uint32_t a0, a1;
+          split2_up(y[j % 2 * 2], up, y[j % 2 * 2 + 1], up, a0, a1);
+          hi[j] = a0;
+          lo[j] = a1;
+        }
+        q.hi[c][s][h] = __builtin_bit_cast(f16x8, hi);
+        q.lo[c][s][h] = __builtin_bit_cast(f16x8, lo);
+      }
+  }
+  return q;
+}
+
 constexpr int kTiles = 8;                       // of the ring, for all shares together
 constexpr int kWindow = 2048, kWindowSlots = kWindow + kWaves * kWave;  // tokens whose slots are looked up at a time
 constexpr float kQTop = 8300000.f;              // below 127 * 2^16 + 127 * 2^8 + 127
@@ -480,23 +557,31 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* to) {
                  : "m0", "memory");
 }
 
-template <int D>
-__global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a) {
+struct Room {  // LDS of the workgroup
+  char* ring;
+  int* slots;
+  float* merge_rl;
+  int* uneven;  // [kWaves]
+};
+
+// An item, with q as Digits, or as Pieces. True: not computed, its q is uneven (the same for the whole workgroup).
+template <int D, bool PIECES>
+__device__ __forceinline__ bool int8_item(const TreeArgs& a, int item, const Room& room) {
   using T = Tile8<D>;
   constexpr int KT = T::KT, TT = 2, KS = D / 64, DT = D / 16;
-  constexpr int kMerge = kWaves * kWaveRows * kMergeRow<D> * 4;  // the ring holds the results in the end
-  __shared__ __attribute__((aligned(16))) char ring[kTiles * T::kBytes > kMerge ? kTiles * T::kBytes : kMerge];
-  __shared__ int slots[kWindowSlots];
-  __shared__ float merge_rl[kWaves * kWaveRows * 2];
-
-  const int lane = threadIdx.x % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  char* const ring = room.ring;
+  int* const slots = room.slots;
+  int tid = threadIdx.x;
+  if constexpr (PIECES) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // the tiles under way have arrived
+    __syncthreads();
+    asm volatile("" : "+v"(tid)::"memory");  // (formed anew: what both forms shared would be held over the other's loop)
+  }
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int fr = lane % 16, fc = lane / 16;
-  int item, last;
-  block_items(a, blockIdx.y, item, last);
-  for (; item < last; ++item) {
   Work w;
-  if (!work_of(a, blockIdx.x, item, wave, w)) continue;
+  if (!work_of(a, blockIdx.x, item, wave, w)) return false;
   const int ctx = w.ctx, t1 = w.t1;
   const bool idle = kWaveRows * w.rw >= w.rows;  // no rows: helps to bring tiles
 
@@ -544,7 +629,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
   auto read_ids = [&](int w0) {
 #pragma unroll
     for (int x = 0; x < kWindowSlots / (kWaves * kWave); ++x) {
-      const int t = w0 + x * kWaves * kWave + static_cast<int>(threadIdx.x);
+      const int t = w0 + x * kWaves * kWave + tid;
       ids[x] = -1;
       if (x * kWaves * kWave < kWindow && t < t1) ids[x] = bt[a.bs_shift >= 0 ? t >> a.bs_shift : t / a.bs];
     }
@@ -555,7 +640,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
     __syncthreads();  // the slots and tiles before it are done with
 #pragma unroll
     for (int x = 0; x < kWindowSlots / (kWaves * kWave); ++x) {
-      const int at = x * kWaves * kWave + static_cast<int>(threadIdx.x), t = w0 + at;
+      const int at = x * kWaves * kWave + tid, t = w0 + at;
       const int in_block = a.bs_shift >= 0 ? t & (a.bs - 1) : t % a.bs;
       slots[at] = ids[x] >= 0 && ids[x] < blocks ? static_cast<int>(ids[x]) * a.bs + in_block : -1;
     }
@@ -565,88 +650,105 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
   read_ids(w.t0);
 
   // ---- q: this wavefront's rows as B operands: lane (fr, fc) dims fc D / 4 .. + D / 4 of row fr -------
-  // The rows are read in whole lines, 1 KB a load (read as the lanes need them, a lane's row at a time, they
-  // took 4 us), and change lanes through the half of the ring that is not under way yet.
-  constexpr int LPR = D / 4, kAtOnce = kWave / LPR, kLoads = 16 / kAtOnce;  // lanes of a row, rows of a load
   uint64_t see[kCols];
-  f32x4 x[kCols][kLoads], mult[kCols][kLoads];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    const int first = w.row0 + kWaveRows * w.rw + 16 * c, end = w.row0 + w.rows - 1;
-    see[c] = static_cast<uint64_t>(a.ancestors[w.first + min(first + fr, end) / a.G]);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int row = min(first + j * kAtOnce + lane / LPR, end), node = row / a.G, head = w.kvh * a.G + row % a.G;
-      x[c][j] = reinterpret_cast<const f32x4*>(a.q + (static_cast<int64_t>(w.first + node) * a.Hq + head) * D)[lane % LPR];
-    }
-  }
+  float qs[kCols];  // score = dot * k_scale * qs (log2 units)
 #pragma unroll
   for (int c = 0; c < kCols; ++c)
+    see[c] = static_cast<uint64_t>(a.ancestors[w.first + (w.row0 + min(kWaveRows * w.rw + 16 * c + fr, w.rows - 1)) / a.G]);
+  std::conditional_t<PIECES, Pieces<D>, Digits<D>> q;
+  if constexpr (PIECES) {
+    start_window(w.t0);
+    q = pieces_of<D>(a, w, lane, qs);
+  } else {
+    // The rows are read in whole lines, 1 KB a load (read as the lanes need them, a lane's row at a time, they
+    // took 4 us), and change lanes through the half of the ring that is not under way yet.
+    constexpr int LPR = D / 4, kAtOnce = kWave / LPR, kLoads = 16 / kAtOnce;  // lanes of a row, rows of a load
+    f32x4 x[kCols][kLoads], mult[kCols][kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) mult[c][j] = f32x4{1.f, 1.f, 1.f, 1.f};
-  if (a.q_mult) {
+    for (int c = 0; c < kCols; ++c) {
+      const int first = w.row0 + kWaveRows * w.rw + 16 * c, end = w.row0 + w.rows - 1;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int row = min(first + j * kAtOnce + lane / LPR, end), node = row / a.G, head = w.kvh * a.G + row % a.G;
+        x[c][j] = reinterpret_cast<const f32x4*>(a.q + (static_cast<int64_t>(w.first + node) * a.Hq + head) * D)[lane % LPR];
+      }
+    }
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
+      for (int j = 0; j < kLoads; ++j) mult[c][j] = f32x4{1.f, 1.f, 1.f, 1.f};
+    if (a.q_mult) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int row = min(w.row0 + kWaveRows * w.rw + 16 * c + j * kAtOnce + lane / LPR, w.row0 + w.rows - 1);
+          const int head = w.kvh * a.G + row % a.G;
+          mult[c][j] = reinterpret_cast<const f32x4*>(a.q_mult + static_cast<int64_t>(head) * D)[lane % LPR];
+        }
+    }
+
+    start_window(w.t0);
+
+    bool uneven = false;  // a row of elements too different in size for digits
+    f32x4* const q_lds = reinterpret_cast<f32x4*>(tile_at(half + w.rw));
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      // row r's four dims n at r LPR + (n ^ r): 16 rows' lie in different banks
+#pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int row = min(w.row0 + kWaveRows * w.rw + 16 * c + j * kAtOnce + lane / LPR, w.row0 + w.rows - 1);
-        const int head = w.kvh * a.G + row % a.G;
-        mult[c][j] = reinterpret_cast<const f32x4*>(a.q_mult + static_cast<int64_t>(head) * D)[lane % LPR];
+        const int r = j * kAtOnce + lane / LPR;
+        q_lds[r * LPR + ((lane % LPR) ^ r)] = x[c][j] * mult[c][j];
       }
-  }
-
-  start_window(w.t0);
-
-  u32x4 qd[kCols][KS][3];  // digits, the largest last
-  float qs[kCols];         // score = dot * k_scale * qs (log2 units)
-  f32x4* const q_lds = reinterpret_cast<f32x4*>(tile_at(half + w.rw));
+      __builtin_amdgcn_wave_barrier();
+      float v[D / 4];
+      float top = 0.f, odd = 0.f;
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    // row r's four dims n at r LPR + (n ^ r): 16 rows' lie in different banks
+      for (int i = 0; i < D / 16; ++i) {
+        const f32x4 y = q_lds[fr * LPR + ((fc * (D / 16) + i) ^ fr)];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int r = j * kAtOnce + lane / LPR;
-      q_lds[r * LPR + ((lane % LPR) ^ r)] = x[c][j] * mult[c][j];
+        for (int e = 0; e < 4; ++e) {
+          v[4 * i + e] = y[e];
+          top = fmaxf(top, fabsf(y[e]));
+          odd = __builtin_fmaf(y[e], 0.f, odd);  // NaN where q is not finite
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      top = max_over_fc(top);
+      odd = sum_over_fc(odd);
+      int bits = 0;  // of the elements' exponents
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) bits += __builtin_amdgcn_frexp_expf(v[i]);
+      uneven |= __ballot(D * __builtin_amdgcn_frexp_expf(top) - sum_over_fc(static_cast<float>(bits)) > kEven * D) != 0;
+      const float f = fminf(kQTop / top, 1e37f);  // (0: 1e37)
+      // the sign of the softmax scale goes with q, so that the scores' order is the dots'; qs > 0: -inf * 0 below
+      const float up = __builtin_copysignf(f, a.scale);
+      qs[c] = fmaxf(fabsf(a.scale) * kLog2e / f, 1e-37f) + odd;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // n + 0x808080 has the digits, each plus 128, as its bytes: the bytes of four elements transposed
+          uint32_t m[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            m[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v[16 * s + 4 * i + e] * up)) + 0x808080);
+          const uint32_t p01 = __builtin_amdgcn_perm(m[1], m[0], 0x05010400u), p23 = __builtin_amdgcn_perm(m[3], m[2], 0x05010400u);
+          const uint32_t h01 = __builtin_amdgcn_perm(m[1], m[0], 0x07030602u), h23 = __builtin_amdgcn_perm(m[3], m[2], 0x07030602u);
+          const uint32_t digit[3] = {__builtin_amdgcn_perm(p23, p01, 0x05040100u) ^ 0x80808080u,
+                                     __builtin_amdgcn_perm(p23, p01, 0x07060302u) ^ 0x80808080u,
+                                     __builtin_amdgcn_perm(h23, h01, 0x05040100u) ^ 0x80808080u};
+#pragma unroll
+          for (int g = 0; g < 3; ++g) q.d[c][s][g][i] = digit[g];
+        }
     }
-    __builtin_amdgcn_wave_barrier();
-    float v[D / 4];
-    float top = 0.f, odd = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const f32x4 y = q_lds[fr * LPR + ((fc * (D / 16) + i) ^ fr)];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[4 * i + e] = y[e];
-        top = fmaxf(top, fabsf(y[e]));
-        odd = __builtin_fmaf(y[e], 0.f, odd);  // NaN where q is not finite
-      }
+    if (w.RW > 1) {  // the same for the whole workgroup (without row groups all have the same rows)
+      if (lane == 0) room.uneven[wave] = uneven;
+      __syncthreads();
+      uneven = __builtin_amdgcn_readfirstlane(room.uneven[0] | room.uneven[1] | room.uneven[2] | room.uneven[3]) != 0;
     }
-    __builtin_amdgcn_wave_barrier();
-    top = max_over_fc(top);
-    odd = sum_over_fc(odd);
-    const float f = fminf(kQTop / top, 1e37f);  // (0: 1e37)
-    // the sign of the softmax scale goes with q, so that the scores' order is the dots'; qs > 0: -inf * 0 below
-    const float up = __builtin_copysignf(f, a.scale);
-    qs[c] = fmaxf(fabsf(a.scale) * kLog2e / f, 1e-37f) + odd;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // n + 0x808080 has the digits, each plus 128, as its bytes: the bytes of four elements transposed
-        uint32_t m[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          m[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v[16 * s + 4 * i + e] * up)) + 0x808080);
-        const uint32_t p01 = __builtin_amdgcn_perm(m[1], m[0], 0x05010400u), p23 = __builtin_amdgcn_perm(m[3], m[2], 0x05010400u);
-        const uint32_t h01 = __builtin_amdgcn_perm(m[1], m[0], 0x07030602u), h23 = __builtin_amdgcn_perm(m[3], m[2], 0x07030602u);
-        const uint32_t digit[3] = {__builtin_amdgcn_perm(p23, p01, 0x05040100u) ^ 0x80808080u,
-                                   __builtin_amdgcn_perm(p23, p01, 0x07060302u) ^ 0x80808080u,
-                                   __builtin_amdgcn_perm(h23, h01, 0x05040100u) ^ 0x80808080u};
-#pragma unroll
-        for (int g = 0; g < 3; ++g) qd[c][s][g][i] = digit[g];
-      }
+    if (uneven) return true;
   }
-
 
   Rows<DT> o;
 #pragma unroll
@@ -680,28 +782,50 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
     }
     __builtin_amdgcn_sched_barrier(0);
     // ---- scores: lane (fr, fc) gets tokens 16 tt + 4 fc + e of its rows
+    if constexpr (!PIECES) {
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      const f32x4 kk_magic = kk[tt] * kMagic;
-      i32x4 dot[kCols][3] = {};
+      for (int tt = 0; tt < TT; ++tt) {
+        const f32x4 kk_magic = kk[tt] * kMagic;
+        i32x4 dot[kCols][3] = {};
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) dot[c][0] = i32x4{kMagicBits, kMagicBits, kMagicBits, kMagicBits};
+        for (int c = 0; c < kCols; ++c) dot[c][0] = i32x4{kMagicBits, kMagicBits, kMagicBits, kMagicBits};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-        for (int g = 0; g < 3; ++g)
+          for (int g = 0; g < 3; ++g)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            dot[c][g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[tt][ks], __builtin_bit_cast(i32x4, qd[c][ks][g]), dot[c][g], 0, 0, 0);
-      }
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int high = (dot[c][2][e] << 8) + dot[c][1][e], low = dot[c][0][e];
-          s[c][tt][e] = __builtin_fmaf(__builtin_fmaf(static_cast<float>(high), 256.f, __builtin_bit_cast(float, low)),
-                                       kk[tt][e], -kk_magic[e]);
+            for (int c = 0; c < kCols; ++c)
+              dot[c][g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[tt][ks], __builtin_bit_cast(i32x4, q.d[c][ks][g]), dot[c][g], 0, 0, 0);
         }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int high = (dot[c][2][e] << 8) + dot[c][1][e], low = dot[c][0][e];
+            s[c][tt][e] = __builtin_fmaf(__builtin_fmaf(static_cast<float>(high), 256.f, __builtin_bit_cast(float, low)),
+                                         kk[tt][e], -kk_magic[e]);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        f32x4 high[kCols] = {}, low[kCols] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x2 x = codes_to_h2(static_cast<uint32_t>(k[tt][ks][2 * h])), y = codes_to_h2(static_cast<uint32_t>(k[tt][ks][2 * h + 1]));
+            const f16x8 kf = __builtin_bit_cast(f16x8, u32x4{x[0], x[1], y[0], y[1]});
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) low[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.lo[c][ks][h], low[c], 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) high[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.hi[c][ks][h], high[c], 0, 0, 0);
+          }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[c][tt][e] = __builtin_fmaf(low[c][e], 1.f / kLoUp, high[c][e]) * kk[tt][e];
+      }
     }
     uint32_t y[8][D / 64];  // V: dims fr D / 16 .. of tokens 4 fc + e and 16 + 4 fc + e
 #pragma unroll
@@ -767,7 +891,30 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
   }
   __syncthreads();
   o.unscale = kVUp;
-  finish<int8_t, D, KT>(a, w, o, reinterpret_cast<float*>(ring), merge_rl, item);
+  finish<int8_t, D, KT>(a, w, o, reinterpret_cast<float*>(ring), room.merge_rl, item);
+  return false;
+}
+
+template <int D>
+__global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a) {
+  using T = Tile8<D>;
+  constexpr int kMerge = kWaves * kWaveRows * kMergeRow<D> * 4;  // the ring holds the results in the end
+  __shared__ __attribute__((aligned(16))) char ring[kTiles * T::kBytes > kMerge ? kTiles * T::kBytes : kMerge];
+  __shared__ int slots[kWindowSlots];
+  __shared__ float merge_rl[kWaves * kWaveRows * 2];
+  __shared__ int uneven[kWaves];
+  const Room room{ring, slots, merge_rl, uneven};
+  int first, last;
+  block_items(a, blockIdx.y, first, last);
+  // The items with uneven q come after the others: in one loop, what the two forms hold is spilled (56 us for 16 trees, in
+  // loops of their own 49). Bits of the items; those past the 31st share one, and are all computed (again) in pieces.
+  uint32_t todo = 0;
+  for (int item = first; item < last; ++item)
+    if (int8_item<D, false>(a, item, room)) todo |= 1u << min(item - first, 31);
+  todo = __builtin_amdgcn_readfirstlane(todo);
+  for (; todo; todo &= todo - 1) {
+    const int i = __builtin_ctz(todo);
+    for (int item = first + i; item < (i < 31 ? first + i + 1 : last); ++item) int8_item<D, true>(a, item, room);
   }
 }
 
@@ -783,7 +930,6 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void tree_int8_kernel(TreeArgs a)
 // with the tokens of a product step side by side, so that no wavefront transposes. Addresses in the loop are formed
 // anew for every tile: kept, they were spilled, and reading them back waits for the rows under way (57 us instead
 // of 47). Rows that are not finite leave NaN in the sums, and plain_rows takes over.
-constexpr int kPieceTop = 15;            // a row's largest value lies in [2^14, 2^15)
 constexpr float kVPieceUp = 1024.f;      // of that, what the weights do not take back (p v_scale lies near 2^kTop with V near 2^5)
 template <int D>
 __global__ __launch_bounds__(kWaves* kWave, 2) void tree_split_kernel(TreeArgs a) {

@@ -211,3 +211,61 @@ def test_sums_over_a_row_in_a_graph(gpu):
         for a, w in ((got.accepted, eager[i].accepted), (got.path, eager[i].path), (got.tokens, eager[i].tokens)):
             assert torch.equal(a, w)
         sp.verify_draft(x, b.draft, tokens, *numbers)
+
+
+@pytest.mark.parametrize("hq,d,nodes", [(2, 128, [24]), (4, 64, [24, 3]), (16, 128, [24, 40]), (32, 64, [64, 1, 7])])
+@pytest.mark.parametrize("size", [30.0, 1e3, 1e5])
+@pytest.mark.parametrize("rows", ["all", "some"])
+@pytest.mark.parametrize("share", [0.0, 0.4])
+def test_queries_of_uneven_channels_over_int8(gpu, hq, d, nodes, size, rows, share):
+    """A channel of q, or a share of them, `size` times the others where K's codes are as much smaller, so that every score is a sum of products of
+    one size; in all nodes or in one of each tree. A float32 product's rounding is relative to each term: every node is
+    as near as with even channels."""
+    b = Batch(47, [333, 90, 2][: len(nodes)], [random_tree(np.random.default_rng(6 + n), n) for n in nodes], 16, gpu, heads=(hq, 2))
+    shape = (b.blocks * b.bs, 2, d)
+    k = b.rng.standard_normal(shape).astype(F32)
+    at = [7] if not share else np.flatnonzero(b.rng.random(d) < share)
+    k[..., at] /= F32(size)
+    (kc, vc), (_, v) = b.caches(d, "int8")
+    idx = torch.arange(len(k), device=gpu)
+    kc.write(idx, torch.from_numpy(k).to(gpu))
+    kc.set_smoothing(torch.ones(2, d), hq)
+    k = kc.rows(idx).cpu().numpy()
+    q = b.rng.standard_normal((b.T, hq, d)).astype(F32)
+    big = np.arange(b.T) if rows == "all" else b.start[:-1] + np.array(nodes) // 2
+    q[np.ix_(big, range(hq), at)] *= F32(size)
+    out = sp.tree_attention(b.put(q, F32), kc, vc, b.draft, d ** -0.5).cpu().numpy().astype(np.float64)
+    want = b.attend64(q, k, v, (kc, vc), d ** -0.5)
+    error = np.linalg.norm(out - want, axis=(1, 2)) / np.linalg.norm(want, axis=(1, 2))
+    assert (error <= 2e-6).all(), (error.argmax(), error.max())
+
+
+def test_uneven_queries_of_very_many_short_sequences(gpu):
+    """Tens of sequences to a workgroup, a few of them with uneven queries."""
+    n, d, rng = 20000, 64, np.random.default_rng(48)
+    b = Batch(48, rng.integers(0, 4, n).tolist(), [[-1]] * n, 4, gpu, heads=(4, 2), max_nodes=1)
+    (kc, vc), (k, v) = b.caches(d, "int8")
+    kc.data[..., 7] = 0
+    k[..., 7] = 0
+    q = rng.standard_normal((n, 4, d)).astype(F32)
+    q[5::97, :, 7] *= 1e4
+    out = sp.tree_attention(b.put(q, F32), kc, vc, b.draft, 0.125).cpu().numpy().astype(np.float64)
+    want = b.attend64(q, k, v, (kc, vc), 0.125)
+    error = np.linalg.norm(out - want, axis=(1, 2)) / np.linalg.norm(want, axis=(1, 2))
+    assert (error <= 2e-6).all(), (error.argmax(), error.max())
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp32"])
+@pytest.mark.parametrize("hq,d", [(2, 128), (16, 128), (4, 64)])
+def test_queries_that_are_not_finite_stay_in_their_rows(gpu, kind, hq, d):
+    """A NaN or an infinity in a node's query makes that row of that head NaN, and no other."""
+    b = Batch(49, [150], [random_tree(np.random.default_rng(3), 24)], 16, gpu, heads=(hq, 2))
+    caches, (k, v) = b.caches(d, kind)
+    q = b.rng.standard_normal((b.T, hq, d)).astype(F32)
+    want = b.attend64(q, k, v, caches, d ** -0.5)
+    odd = np.zeros((b.T, hq), bool)
+    for node, head, value in ((0, 0, np.nan), (5, hq - 1, np.inf), (23, 0, -np.inf)):
+        q[node, head, 9], odd[node, head] = value, True
+    out = sp.tree_attention(b.put(q, F32), *caches, b.draft, d ** -0.5).cpu().numpy().astype(np.float64)
+    assert np.isnan(out[odd]).all() and np.isfinite(out[~odd]).all()
+    assert np.linalg.norm(out[~odd] - want[~odd]) <= 2e-6 * np.linalg.norm(want[~odd])
