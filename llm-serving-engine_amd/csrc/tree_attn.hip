@@ -26,10 +26,10 @@
 // each channel's.
 //
 // What bounds it. int8, 32 trees of up to 64 nodes over 1K to 8K tokens (1716 nodes, 16 heads, 8 of K/V, D 128, 55 GFLOP,
-// 298 MB): 166 us, 330 TFLOP/s; vector instructions (13 for each score of a lane, 80 to widen V) are issued in 64 % of the
+// 298 MB): 168 us, 330 TFLOP/s; vector instructions (13 for each score of a lane, 80 to widen V) are issued in 64 % of the
 // SIMDs' cycles, the matrix unit is busy in 31 %, hidden behind them. 16 trees of 26 nodes: 46 us, 1.9 TB/s: 22 us
 // of tiles, the rest the starts and ends of the workgroups (plan, table, q: 8 us, joining 4 us) and the second launch
-// (61 % and 22 %). One stream: 16 us of kernels, two launches and one tile. Single tokens of 64
+// (61 % and 21 %). One stream: 16 us of kernels, two launches and one tile. Single tokens of 64
 // sequences over 2K tokens: 78 us, 3.5 TB/s. fp32: 32 sequences of 5 nodes (10 rows) over 1K to 4K tokens 136 us, 4.9 TB/s; 208
 // rows a kv head 46 us (95 TFLOP/s) in fp16 pieces, vector instructions in 49 %, products in 18 % of the cycles. D 64, 16
 // trees of 26 nodes over 512 to 4K tokens, 8 kv heads: int8 29 us, 1.5 TB/s, fp32 46 us, 3.5 TB/s.
